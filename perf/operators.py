@@ -12,7 +12,6 @@ even column) times its block's scale:
 both rounded to the nearest, ties to the even code, magnitudes above 6 to 6.
 """
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -27,14 +26,12 @@ DTYPES = {"bfloat16": torch.bfloat16, "float16": torch.float16, "float32": torch
 DEVICE = "cuda"
 
 
-@functools.cache
 def _fp4():
     _package()
     from wan_dit_lab_b200.quantization import fp4
     return fp4
 
 
-@functools.cache
 def _gated_norm():
     _package()
     from wan_dit_lab_b200.kernels.gated_norm import gated_norm
