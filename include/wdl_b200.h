@@ -421,6 +421,11 @@ int wdl_fp4_dequantize_rows(const uint8_t* codes, const uint8_t* scales, int M, 
 int wdl_fp4_gemm(const wdl_fp4_rows* a, const wdl_fp4_rows* w, const float* bias, int M, int N, int K, void* out,
                  int out_dtype, int64_t ldo, void* stream);
 
+/* Which kernel a product of these sizes takes on a GPU with `sms` multiprocessors: 0 the one for many rows, else the rows of a
+ * that one CTA of the few-row kernel takes (16, 64 or 128); -1 for sizes that are not positive. Results do not depend on
+ * it but for the order of float32 sums. */
+int wdl_fp4_gemm_rows_per_cta(int M, int N, int K, int sms);
+
 /* out [M, N] f32 = residual + gate * (a w^T + bias): the gated residual update of a block. gate [groups, ld_gate] f32
  * (nullable: 1): row m takes group m / (M / groups), M a multiple of groups. out may be residual itself (the same
  * rows), and otherwise overlaps nothing that is read. */

@@ -322,3 +322,15 @@ def test_packed_layers_refuse(fake):
         fp4.PackedFp4Linear(cuda(8, 32, dtype=torch.uint8), cuda(8, 3, dtype=torch.uint8))
     with pytest.raises(ValueError, match="unknown FP4 format"):
         fp4.quantize(cuda(8, 64), fmt="fp6")
+
+
+def test_every_product_kernel_has_its_sizes():
+    """The rule by which a product's kernel is chosen, for 148 multiprocessors, on either side of its borders."""
+    from wan_dit_lab_b200 import _native
+    rows = _native.lib().wdl_fp4_gemm_rows_per_cta
+    for sizes, want in [((1, 1 << 20, 32), 16), ((16, 64, 64), 16), ((17, 64, 64), 64), ((64, 1 << 20, 1 << 20), 64),
+                        ((65, 98 * 64, 3072), 64), ((65, 99 * 64, 3072), 0), ((65, 32 * 128, 9024), 64), ((65, 33 * 128, 9024), 128),
+                        ((1100, 700, 3840), 0), ((1100, 700, 3872), 128), ((128, 88 * 128, 4096), 128), ((128, 89 * 128, 4096), 0),
+                        ((2 ** 31 - 2 ** 16, 2 ** 31 - 2 ** 16, 64), 0), ((0, 8, 64), -1), ((8, 0, 64), -1), ((8, 8, 0), -1)]:
+        assert rows(*sizes, 148) == want, sizes
+    assert rows(8, 8, 64, 0) == -1

@@ -1,0 +1,166 @@
+"""The FP4 products of many rows (gemm_pair_kernel) and of many rows over long K (the 128-row CTAs of gemm_few_kernel) against
+the oracle. Every test asks the library which kernel its sizes take, so that another rule leaves no kernel untested."""
+
+import numpy as np
+import pytest
+import test_fp4_gpu as small
+import torch
+from test_fp4_gpu import DEV, DTYPES, FORMATS, activations, generator, product_tolerance, weight_rows
+
+from oracle import fp4 as oracle
+
+pytestmark = pytest.mark.gpu
+
+
+def takes(rows_per_cta, M, N, K):
+    """The sizes take the kernel that the test is about."""
+    from wan_dit_lab_b200 import _native
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert _native.lib().wdl_fp4_gemm_rows_per_cta(M, N, K, sms) == rows_per_cta
+
+
+# one tile a pair and several, a last tile of few rows or features, K that ends inside a stage at each of its steps of 64
+# and inside one, one stage and more than the ring holds
+MANY = [(3300, 261, 288), (3300, 258, 160), (4700, 1288, 96), (520, 1416, 544), (1030, 900, 1312),
+        (6500, 33, 2080), (2049, 513, 512), (1700, 512, 3808)]
+LONG = [(1100, 700, 4128), (1500, 390, 9024), (1153, 704, 3872)]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", MANY)
+def test_linear_of_many_rows(fmt, M, N, K):
+    takes(0, M, N, K)
+    small.test_linear_against_float64(fmt, M, N, K)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", LONG)
+def test_linear_of_many_rows_over_long_k(fmt, M, N, K):
+    takes(128, M, N, K)
+    small.test_linear_against_float64(fmt, M, N, K)
+
+
+@pytest.mark.parametrize("kernel,M,N,K,groups", [
+    (0, 3300, 264, 288, 1), (0, 3300, 261, 96, 11), (0, 4700, 1288, 64, 5), (0, 3300, 258, 160, 3300), (0, 2050, 516, 320, 2),
+    (128, 1100, 700, 4128, 4), (128, 1152, 701, 3872, 9)])
+def test_gated_residual_of_many_rows(kernel, M, N, K, groups):
+    """Groups that are whole, that end inside a tile, and of one row; against float64, and strided in place."""
+    takes(kernel, M, N, K)
+    small.test_gated_residual(M, N, K, groups)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", [(3300, 260, 192), (4700, 1284, 192)])
+def test_aligned_residual_in_place(fmt, M, N, K):
+    """The stream read and written through TMA, in place, with one gate, none, and one for groups that end inside a tile."""
+    from wan_dit_lab_b200.quantization import fp4
+    takes(0, M, N, K)
+    x = activations(M, K, 100, torch.bfloat16)
+    w, wv = weight_rows(N, K, fmt, 101)
+    g = generator(102)
+    residual, bias = torch.randn(M, N, generator=g).to(DEV), torch.randn(N, generator=g).to(DEV)
+    a = oracle.rounded(x.float().cpu().numpy(), fmt).astype(np.float64)
+    y = a @ wv.T + bias.double().cpu().numpy()
+    tol = product_tolerance(a, wv, y, torch.float32)
+    for gate in (None, torch.randn(N, generator=g).to(DEV), torch.randn(10, N, generator=g).to(DEV)):
+        rows = np.ones((1, 1)) if gate is None else np.repeat(gate.double().cpu().numpy().reshape(-1, N),
+                                                               M // (1 if gate.ndim == 1 else 10), axis=0)
+        stream = residual.clone()
+        assert fp4.fp4_linear(x, w, bias, residual=stream, gate=gate, out=stream) is stream
+        want = residual.double().cpu().numpy() + rows * y
+        # the fused multiply-add rounds once
+        assert (np.abs(stream.double().cpu().numpy() - want) <= np.abs(rows) * tol + 2.0 ** -24 * 1.01 * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("kernel,M,N", [(0, 3300, 258), (0, 4700, 1285), (0, 7000, 31)])
+def test_residual_of_many_rows_that_begin_anywhere(kernel, M, N):
+    takes(kernel, M, N, 192)
+    small.test_gated_residual_with_rows_that_begin_anywhere(M, N)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("first,second,M,K,H,N", [
+    (0, 0, 3300, 96, 288, 264), (0, 0, 4700, 288, 1056, 264), (0, 0, 2050, 64, 544, 513), (128, 0, 1100, 4128, 704, 800),
+    (0, 128, 1100, 96, 4128, 700)])
+def test_gelu_mlp_of_many_rows(fmt, first, second, M, K, H, N):
+    """The hidden layer's codes and scales, the last tile's padding among them, and the second product of them."""
+    takes(first, M, H, K)
+    takes(second, M, N, H)
+    small.test_gelu_mlp(fmt, M, K, H, N)
+
+
+@pytest.mark.parametrize("M", [1700, 1665])
+def test_a_square_layer_of_many_rows_onto_its_own_input(M):
+    takes(0, M, 512, 512)
+    small.test_a_square_layer_onto_its_own_input(M)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("bad", [float("nan"), -float("inf")])
+def test_non_finite_values_stay_in_their_rows_of_many(fmt, bad):
+    from wan_dit_lab_b200.quantization import fp4
+    M, N, K = 3300, 264, 288
+    takes(0, M, N, K)
+    x = activations(M, K, 110)
+    rows = torch.tensor([0, 127, 128, 300, 3299], device=DEV)
+    x[rows, torch.tensor([0, 31, 255, 256, 287], device=DEV)] = bad
+    w, _ = weight_rows(N, K, fmt, 111)
+    other = torch.ones(M, dtype=torch.bool, device=DEV)
+    other[rows] = False
+    nan = fp4.fp4_linear(x, w, dtype=torch.float32).isnan()
+    assert nan[rows].all() and not nan[other].any()
+    w2, _ = weight_rows(N, N + 24, fmt, 112)
+    w1, _ = weight_rows(N + 24, K, fmt, 113)
+    nan = fp4.fp4_gelu_mlp(x, w1, None, w2, None, residual=torch.zeros(M, N, device=DEV)).isnan()
+    assert nan[rows].all() and not nan[other].any()
+
+
+def test_many_rows_on_other_streams_and_in_graphs():
+    """Both products of a feed forward with many rows: on a side stream, and in two graphs replayed in turn."""
+    from wan_dit_lab_b200 import _native
+    from wan_dit_lab_b200.quantization import fp4
+    M, D, H = 3300, 288, 1056
+    takes(0, M, H, D)
+    takes(0, M, D, H)
+    w1, _ = weight_rows(H, D, "nvfp4", 120)
+    w2, _ = weight_rows(D, H, "nvfp4", 121)
+    x = activations(M, D, 122)
+    want = [fp4.fp4_gelu_mlp(x * k, w1, None, w2, None, residual=x * k) for k in (1, 2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [fp4.fp4_gelu_mlp(x, w1, None, w2, None, residual=x) for _ in range(10)]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(y, want[0]) for y in got)
+    graphs = []
+    for _ in range(2):
+        static = x.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = fp4.fp4_gelu_mlp(static, w1, None, w2, None, residual=static)
+        graphs.append((graph, static, out))
+    for k in (1, 2, 1):
+        for graph, static, out in graphs:
+            static.copy_(x * k)
+            graph.replay()
+            assert torch.equal(out, want[k - 1])
+    assert _native.device_error() == 0
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_weights_made_just_before_a_product_of_many_rows(fmt):
+    from wan_dit_lab_b200.quantization import fp4
+    M, N, K = 1700, 1024, 1056
+    takes(0, M, N, K)
+    x = activations(M, K, 130, torch.bfloat16)
+    W = [torch.randn(N, K, generator=generator(131 + i)).to(DEV) * 0.02 for i in range(4)]
+    q = fp4.quantize_rows(x, fmt)
+    want = [fp4.fp4_linear(q, fp4.quantize_rows(w, fmt)) for w in W]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for w in W:
+            got.append(fp4.fp4_linear(q, fp4.quantize_rows(w, fmt)))
+            got.append(fp4.fp4_linear(x, fp4.quantize_rows(w, fmt)))
+        for i in range(4):
+            assert torch.equal(got[2 * i], want[i]) and torch.equal(got[2 * i + 1], want[i])

@@ -64,6 +64,8 @@ struct GemmArgs {
   Epilogue ep;
   uint32_t* err;
 };
+// Rows of a that one CTA of the few-row kernel takes, 0 for the many-row kernel (which does not split K).
+int gemm_rows_per_cta(int M, int N, int K, int sms);
 // Validated by the caller. 0, or nonzero with *why set.
 int gemm_launch(const GemmArgs& a, cudaStream_t s, const char** why);
 

@@ -81,6 +81,10 @@ int wdl_fp4_dequantize_rows(const uint8_t* codes, const uint8_t* scales, int M, 
                                                       static_cast<cudaStream_t>(stream)));
 }
 
+int wdl_fp4_gemm_rows_per_cta(int M, int N, int K, int sms) {
+  return M <= 0 || N <= 0 || K <= 0 || sms <= 0 ? -1 : wdl::fp4::gemm_rows_per_cta(M, N, K, sms);
+}
+
 static int run_gemm(wdl::fp4::GemmArgs& g, const wdl_fp4_rows* a, const wdl_fp4_rows* w, const float* bias, int M, int N,
                     int K, bool early_w, void* stream) {
   if (!a || !w) return refuse("null operand");

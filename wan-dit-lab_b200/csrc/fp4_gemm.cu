@@ -1168,22 +1168,24 @@ static bool make_maps(Maps& m, const GemmArgs& g, int few) {
   return ok;
 }
 
+// Up to 64 rows the few-row kernel is the faster one (N 14336, K 3072: 8.2 against 8.9 us at 64 rows, 9.5 against 8.5 at
+// 96). Beyond, 64 rows a CTA where these are few enough for K to be split, two thirds of the SMs (128 rows: 4.4 against 5.5
+// us for N 512, K 1024, 7.2 against 7.9 for N 3072, K 3072, 5.7 against 13.2 for N 512, K 8192; 256 rows, 96 CTAs: 7.7
+// against 7.9 for N 3072, K 3072). Where K is long, at most half as many: CTAs of 128 rows read w less often (K 14336, N
+// 3072: 10.9 against 12.0 us at 128 rows, 13.7 against 13.0 at 160), and are taken as long as their parts find room beside
+// each other (18.1 against the many-row kernel's 21.5 us at 384 rows, 22.2 against 21.5 at 512).
+int gemm_rows_per_cta(int M, int N, int K, int sms) {
+  const int64_t n128 = (static_cast<int64_t>(N) + 127) / 128, tiles64 = (static_cast<int64_t>(M) + 63) / 64 * n128;
+  const int64_t tiles128 = (static_cast<int64_t>(M) + 127) / 128 * n128;
+  if (M <= 16) return 16;
+  if (M <= 64 || tiles64 * (K > 8192 ? 3 : 2) * 3 <= sms * 4) return 64;
+  return K > 15 * BK && tiles128 * 3 <= sms * 9 / 5 ? 128 : 0;
+}
+
 int gemm_launch(const GemmArgs& g, cudaStream_t s, const char** why) {
   Device d{0, 148};
   if (cudaGetDevice(&d.id) == cudaSuccess) cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, d.id);
-  // Rows of a that one few-row CTA takes, 0 for the many-row kernel, which does not split K. Up to 64 rows the few-row kernel
-  // is the faster one (N 14336, K 3072: 8.2 against 8.9 us at 64 rows, 9.5 against 8.5 at 96). Beyond, 64 rows a CTA where
-  // these are few enough for K to be split, two thirds of the SMs (128 rows: 4.4 against 5.5 us for N 512, K 1024, 7.2
-  // against 7.9 for N 3072, K 3072, 5.7 against 13.2 for N 512, K 8192; 256 rows, 96 CTAs: 7.7 against 7.9 for N 3072,
-  // K 3072). Where K is long, at most half as many: CTAs of 128 rows read w less often (K 14336, N 3072: 10.9 against 12.0
-  // us at 128 rows, 13.7 against 13.0 at 160), and are taken as long as their parts find room beside each other (18.1
-  // against the many-row kernel's 21.5 us at 384 rows, 22.2 against 21.5 at 512).
-  const int64_t n128 = (g.N + 127) / 128, tiles64 = (static_cast<int64_t>(g.M) + 63) / 64 * n128;
-  const int64_t tiles128 = (static_cast<int64_t>(g.M) + 127) / 128 * n128;
-  const int few = g.M <= 16                                                     ? 16
-                  : g.M <= 64 || tiles64 * (g.K > 8192 ? 3 : 2) * 3 <= d.sms * 4 ? 64
-                  : g.K > 15 * BK && tiles128 * 3 <= d.sms * 9 / 5               ? 128
-                                                                                 : 0;
+  const int few = gemm_rows_per_cta(g.M, g.N, g.K, d.sms);
   Maps m{};
   if (!make_maps(m, g, few)) {
     *why = "cuTensorMapEncodeTiled rejected an operand (alignment or stride)";

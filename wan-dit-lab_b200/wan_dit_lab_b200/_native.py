@@ -95,6 +95,7 @@ SIGNATURES = {
     "wdl_fp4_quantize_rows": (_I, [_P, _I, _I64, _I, _I, _I, _P, _P, _P, _P]),
     "wdl_fp4_dequantize_rows": (_I, [_P, _P, _I, _I, _I, _P, _P, _I, _I64, _P]),
     "wdl_fp4_gemm": (_I, [_PACKED, _PACKED, _P, _I, _I, _I, _P, _I, _I64, _P]),
+    "wdl_fp4_gemm_rows_per_cta": (_I, [_I, _I, _I, _I]),
     "wdl_fp4_gemm_residual": (_I, [_PACKED, _PACKED, _P, _P, _I, _I64, _P, _I64, _I, _I, _I, _P, _I64, _P]),
     "wdl_fp4_gemm_gelu": (_I, [_PACKED, _PACKED, _P, _I, _I, _I, _P, _P, _P, _P]),
     "wdl_fp4_linear_workspace": (_SZ, [_I, _I, _I]),
