@@ -79,6 +79,16 @@ def test_residual_of_many_rows_that_begin_anywhere(kernel, M, N):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N", [(4700, 167), (3300, 261), (4700, 1191), (4700, 1290)])
+def test_outputs_of_many_rows_that_begin_anywhere(fmt, M, N):
+    """Every alignment of rows; among them rows that TMA stores up to a last group of columns that ends off a 16-byte
+    boundary, which the warp stores itself, in between (float32, N 167 and rows of 168)."""
+    takes(0, M, N, 192)
+    for _ in range(3):
+        small.test_outputs_that_begin_anywhere(fmt, M, N)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("first,second,M,K,H,N", [
     (0, 0, 3300, 96, 288, 264), (0, 0, 4700, 288, 1056, 264), (0, 0, 2050, 64, 544, 513), (128, 0, 1100, 4128, 704, 800),
     (0, 128, 1100, 96, 4128, 700)])

@@ -615,6 +615,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               store_words<kMode>(buf, ep.out, ep.ld_out, lane, m0, x, M, N);
               fence_proxy_async_smem();
               __syncwarp();
+              if (lane == 0) bulk_commit();  // an empty group: the waits count a group for every use of a buffer
             }
             if constexpr (kMode == kEpiResidual)
               if (staged) load_residual();
