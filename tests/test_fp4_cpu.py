@@ -206,6 +206,18 @@ def test_rows_that_overlap():
         assert overlaps(out, t) is want, (out.shape, t.shape)
 
 
+def test_only_all_of_the_same_rows_are_updated_in_place():
+    """A part of the rows, or what is no residual, overlaps even where it begins at the same address."""
+    from wan_dit_lab_b200._native import overlaps
+    b = torch.zeros(10, 64)
+    for out, t, in_place, want in [
+            (b, b, True, False), (b, b[:3], True, True), (b[:3], b, True, True), (b, b[0], True, True),
+            (b, b[:, :32], True, True), (b[:, :32], b, True, True), (b[:1], b[0, :32], True, True), (b[:5], b[5:], False, False),
+            (b, b, False, True), (b[:1], b[0], False, True), (b[:1], b[:1], False, True), (b[:, :32], b[:, 32:], False, False),
+            (b[::2], b[1::2], False, False), (b[::2], b[::2], False, True), (b[:1], b[1], False, False)]:
+        assert overlaps(out, t, in_place) is want, (out.shape, t.shape, in_place)
+
+
 @pytest.fixture
 def fake(monkeypatch):
     from wan_dit_lab_b200 import _native

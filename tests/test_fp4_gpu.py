@@ -573,3 +573,25 @@ def test_rows_in_blocks_of_64(fmt, M, N, K):
     residual = torch.randn(M, N, generator=generator(92)).to(DEV)
     z = fp4.fp4_linear(q, w, residual=residual)
     assert (z - (residual + y)).abs().max() <= 2.0 ** -22 * (residual.abs() + y.abs()).max()  # another order of two roundings
+
+
+def test_modulation_out_of_the_output_itself_is_refused():
+    """gate, bias, weight, shift and scale that are the output's first rows, or a single row's own."""
+    from wan_dit_lab_b200.kernels.gated_norm import gated_norm
+    from wan_dit_lab_b200.quantization import fp4
+    w, _ = weight_rows(64, 64, "nvfp4", 140)
+    for M in (1, 6):
+        x = activations(M, 64, 141)
+        r = torch.randn(M, 64, generator=generator(142)).to(DEV)
+        keep = r.clone()
+        for wrong in (dict(gate=r[:1]), dict(gate=r[0]), dict(gate=r[:M // 2 or 1]), dict(gate=r), dict(bias=r[0])):
+            with pytest.raises(ValueError, match="overlap"):
+                fp4.fp4_linear(x, w, residual=r, out=r, **wrong)
+        for wrong in (dict(gate=r[:1]), dict(shift=r[0]), dict(scale=r[:M // 2 or 1]), dict(weight=r[0]), dict(bias=r[0]),
+                      dict(gate=r)):
+            with pytest.raises(ValueError, match="overlap"):
+                gated_norm(r, x, inplace=True, **wrong)
+        assert torch.equal(r, keep)
+        # the same rows are what a call that writes elsewhere may read
+        want = fp4.fp4_linear(x, w, r[0].clone(), residual=r, gate=r.clone())
+        assert torch.equal(fp4.fp4_linear(x, w, r[0], residual=r, gate=r), want)

@@ -171,10 +171,11 @@ def flat_rows(x, columns):
     return x.contiguous()
 
 
-def overlaps(out, t):
+def overlaps(out, t, in_place=True):
     """Whether the rows of `t` (a matrix or a vector with consecutive elements) lie in the rows that `out` is about to be
-    written to, without being the very same ones: a kernel reads each element just before it writes that one, so that
-    the same rows are updated in place, and shifted ones are read too late."""
+    written to. in_place: but for the very same rows, all of them. That is right for what a kernel reads element by
+    element just before it writes that one (a residual, a branch); anything else, a modulation row or a bias, is read for
+    other elements too and by then may hold what was written."""
     rows, columns = out.shape
     count, width = t.shape if t.ndim == 2 else (1, t.shape[0])
     if 0 in (rows, columns, count, width):
@@ -185,7 +186,7 @@ def overlaps(out, t):
     if at + (rows - 1) * step + columns * size <= at_t or at_t + (count - 1) * step_t + width * size_t <= at:
         return False
     same = rows == 1 == count or step == step_t
-    if at == at_t and same and out.dtype == t.dtype:
+    if in_place and at == at_t and same and (rows, columns, out.dtype) == (count, width, t.dtype):
         return False
     apart = (at_t - at) % step if same and step else 0  # rows side by side in one buffer
     return not (apart >= columns * size and apart + width * size_t <= step)

@@ -105,7 +105,7 @@ def gated_norm(x, y=None, gate=None, *, weight=None, bias=None, shift=None, scal
         y = _native.rows16(y)
         y_ptr, ldy, y_code = y.data_ptr(), _row_stride(y, K), _native.DTYPE_CODE[y.dtype]
         if inplace:
-            if any(r is not None and _native.overlaps(x, r) for r in (y, g, sh, sc, w, b)):
+            if _native.overlaps(x, y) or any(r is not None and _native.overlaps(x, r, False) for r in (g, sh, sc, w, b)):
                 raise ValueError("what the kernel reads must not overlap an in-place stream (y may be the stream itself)")
         else:
             stored = torch.empty(M, K, dtype=x.dtype, device=dev)

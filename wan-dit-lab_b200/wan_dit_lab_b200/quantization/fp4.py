@@ -281,7 +281,7 @@ def _output(lead, M, N, device, dtype, bias, residual, gate, out):
         flat = out if out.ndim == 2 else out.view(-1, N)
         if N > 1 and flat.stride(1) != 1 or M > 1 and flat.stride(0) < N:
             raise ValueError("out must have consecutive elements in its rows, and rows apart from one another")
-        if any(t is not None and _native.overlaps(flat, t) for t in (res, gate, bias)):
+        if _native.overlaps(flat, res) or any(t is not None and _native.overlaps(flat, t, False) for t in (gate, bias)):
             raise ValueError("out may be the residual itself, but must not overlap it otherwise, nor the gate or the bias")
         ld_out = _row_stride(flat, N)
     return out, flat.data_ptr(), _native.F32, ld_out, (gate_ptr, groups, ld_gate, res.data_ptr(), _row_stride(res, N)), (gate, res)
