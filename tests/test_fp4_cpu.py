@@ -4,6 +4,8 @@ the header, and what the entry points and the Python layer refuse before anythin
 import ctypes
 import itertools
 import re
+import shutil
+import subprocess
 from pathlib import Path
 
 import numpy as np
@@ -346,3 +348,16 @@ def test_every_product_kernel_has_its_sizes():
                         ((2 ** 31 - 2 ** 16, 2 ** 31 - 2 ** 16, 64), 0), ((0, 8, 64), -1), ((8, 0, 64), -1), ((8, 8, 0), -1)]:
         assert rows(*sizes, 148) == want, sizes
     assert rows(8, 8, 64, 0) == -1
+
+
+def test_tiles_of_the_many_row_product(tmp_path):
+    """Every tile is taken once, and nothing undefined is computed for the step past a pair's last tile."""
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("no g++")
+    exe = tmp_path / "fp4_tiles_check"
+    source = Path(__file__).resolve().parent / "native" / "fp4_tiles_check.cpp"
+    subprocess.run([gxx, "-std=c++17", "-O1", "-Wall", "-Wextra", "-Werror", "-fsanitize=undefined", "-fno-sanitize-recover=all",
+                    str(source), "-o", str(exe)], check=True)
+    run = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert run.returncode == 0 and run.stdout == "ok\n", run.stderr

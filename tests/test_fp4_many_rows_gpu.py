@@ -19,9 +19,9 @@ def takes(rows_per_cta, M, N, K):
     assert _native.lib().wdl_fp4_gemm_rows_per_cta(M, N, K, sms) == rows_per_cta
 
 
-# one tile a pair and several, a last tile of few rows or features, K that ends inside a stage at each of its steps of 64
-# and inside one, one stage and more than the ring holds
-MANY = [(3300, 261, 288), (3300, 258, 160), (4700, 1288, 96), (520, 1416, 544), (1030, 900, 1312),
+# one tile a pair and several, a last tile of few rows or features, row pairs a multiple of 8 (the groups of tiles), K that
+# ends inside a stage at each of its steps of 64 and inside one, one stage and more than the ring holds
+MANY = [(3300, 261, 288), (3300, 258, 160), (4700, 1288, 96), (4096, 1288, 64), (520, 1416, 544), (1030, 900, 1312),
         (6500, 33, 2080), (2049, 513, 512), (1700, 512, 3808)]
 LONG = [(1100, 700, 4128), (1500, 390, 9024), (1153, 704, 3872)]
 

@@ -11,6 +11,7 @@
 
 #include "fp4.cuh"
 #include "fp4.h"
+#include "fp4_tiles.h"
 #include "w4a4_gemm.h"
 
 namespace wdl {
@@ -199,16 +200,6 @@ __host__ __device__ constexpr int stage_tiles(int fmt) { return BK / tile_column
 constexpr int store_columns(int mode) { return mode == kEpiF32 || mode == kEpiResidual ? 32 : 64; }
 constexpr int buffer_bytes(int mode) { return mode == kEpiGelu ? 1024 : 4096; }
 constexpr int buffers(int mode) { return mode == kEpiBf16 || mode == kEpiF16 ? 1 : 2; }
-
-// Tile t: row pairs fastest within groups of 8 of them, so that the tiles under way at one time share rows of a as well
-// as of w in L2 however many rows there are.
-struct Tile {
-  int m_pair, n_tile;
-};
-__device__ __forceinline__ Tile tile_of(int t, int m_pairs, int n_tiles) {
-  const int group = t / (8 * n_tiles), rows = min(8, m_pairs - group * 8), r = t - group * 8 * n_tiles;
-  return {group * 8 + r % rows, r / rows};
-}
 
 template <int kFmt, int kMode>
 struct __align__(1024) Smem {
