@@ -174,3 +174,46 @@ def test_weights_made_just_before_a_product_of_many_rows(fmt):
             got.append(fp4.fp4_linear(x, fp4.quantize_rows(w, fmt)))
         for i in range(4):
             assert torch.equal(got[2 * i], want[i]) and torch.equal(got[2 * i + 1], want[i])
+
+
+def test_calls_from_several_threads_at_once():
+    """Threads with streams of their own, every kernel, from each kernel's first launch in a fresh process on (what is asked
+    of the device once is asked by several of them)."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    program = """
+import sys, threading
+sys.path[:0] = {paths!r}
+import torch
+from test_fp4_gpu import activations, weight_rows
+from wan_dit_lab_b200 import _native
+from wan_dit_lab_b200.kernels.gated_norm import gated_norm
+from wan_dit_lab_b200.quantization import fp4
+layers = [weight_rows(N, K, "nvfp4", N)[0] for N, K in ((1056, 288), (288, 1056))]
+xs = [activations(M, 288, M, torch.bfloat16) for M in (1, 9, 40, 3300)]
+torch.cuda.synchronize()
+def call(x):
+    s, rows = gated_norm(x, x, out="nvfp4")
+    y = fp4.fp4_gelu_mlp(rows, layers[0], None, layers[1], None, dtype=torch.float32)
+    return y, fp4.fp4_linear(x, layers[0]), fp4.dequantize_rows(fp4.quantize_rows(x, "mxfp4"))
+start, got = threading.Barrier(4), {{}}
+def work(i):
+    with torch.cuda.stream(torch.cuda.Stream()):
+        start.wait()
+        got[i] = [call(x) for _ in range(20) for x in xs[i:] + xs[:i]]
+        torch.cuda.current_stream().synchronize()
+threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+for t in threads: t.start()
+for t in threads: t.join()
+for i in range(4):
+    for j, out in enumerate(got[i]):
+        for a, b in zip(out, call((xs[i:] + xs[:i])[j % 4])):
+            assert torch.equal(a, b), (i, j)
+assert _native.device_error() == 0
+print("ok")
+"""
+    here = Path(__file__).resolve().parent
+    paths = [str(here.parent / "wan-dit-lab_b200"), str(here.parent), str(here)]
+    run = subprocess.run([sys.executable, "-c", program.format(paths=paths)], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout.strip() == "ok", run.stdout + run.stderr

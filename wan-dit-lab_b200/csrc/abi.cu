@@ -1,5 +1,6 @@
 // The extern "C" entry points of include/wdl_b200.h: argument validation (before any launch or write),
 // status codes and per-thread error messages, the per-device error word, and the tensor-map encoder.
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -38,18 +39,20 @@ bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p
 __device__ uint32_t g_device_error;
 
 constexpr int kMaxDevices = 64;
-uint32_t* g_error_word[kMaxDevices] = {};
+std::atomic<uint32_t*> g_error_word[kMaxDevices] = {};
 
 // Address of this device's error word (resolved once per device, with that device current).
 uint32_t* error_word() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return nullptr;
-  if (!g_error_word[dev]) {
+  uint32_t* word = g_error_word[dev].load(std::memory_order_relaxed);
+  if (!word) {
     void* p = nullptr;
     if (cudaGetSymbolAddress(&p, g_device_error) != cudaSuccess) return nullptr;
-    g_error_word[dev] = static_cast<uint32_t*>(p);
+    word = static_cast<uint32_t*>(p);
+    g_error_word[dev].store(word, std::memory_order_relaxed);
   }
-  return g_error_word[dev];
+  return word;
 }
 
 int cuda_status(cudaError_t e, const char* what) {
@@ -76,7 +79,8 @@ bool encode_tiled(CUtensorMap* map, CUtensorMapDataType dtype, cuuint32_t rank, 
                   const cuuint64_t* strides, const cuuint32_t* box, const cuuint32_t* elem_strides,
                   CUtensorMapInterleave interleave, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion l2,
                   CUtensorMapFloatOOBfill fill) {
-  static EncodeTiledFn fn = nullptr;
+  static std::atomic<EncodeTiledFn> known{nullptr};
+  EncodeTiledFn fn = known.load(std::memory_order_relaxed);
   if (!fn) {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -84,6 +88,7 @@ bool encode_tiled(CUtensorMap* map, CUtensorMapDataType dtype, cuuint32_t rank, 
         q != cudaDriverEntryPointSuccess || !p)
       return false;
     fn = reinterpret_cast<EncodeTiledFn>(p);
+    known.store(fn, std::memory_order_relaxed);
   }
   return fn(map, dtype, rank, base, dims, strides, box, elem_strides, interleave, swizzle, l2, fill) ==
          CUDA_SUCCESS;

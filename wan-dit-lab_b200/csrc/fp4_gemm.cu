@@ -6,6 +6,7 @@
 // shared memory, block scales from TMEM, float32 accumulation of all of K. Nothing is unpacked or promoted.
 //
 // Two kernels: gemm_pair_kernel for many rows of a, gemm_few_kernel for few.
+#include <atomic>
 #include <cstddef>
 #include <type_traits>
 
@@ -1026,13 +1027,14 @@ static bool scales_map(CUtensorMap* map, const uint8_t* scales, int K, int rows,
                   stage_tiles(fmt) * kTileBytes / 8, blocks, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-// The attributes a kernel needs before its first launch on a device, set once per device.
+// The attributes a kernel needs before its first launch on a device, set once per device (by every thread that gets here
+// before the first has: the same values).
 template <typename Kernel>
-static cudaError_t allow_smem(Kernel kernel, int bytes, int dev, bool (&done)[64]) {
-  if (dev >= 0 && dev < 64 && done[dev]) return cudaSuccess;
+static cudaError_t allow_smem(Kernel kernel, int bytes, int dev, std::atomic<bool> (&done)[64]) {
+  if (dev >= 0 && dev < 64 && done[dev].load(std::memory_order_relaxed)) return cudaSuccess;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-  if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+  if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_relaxed);
   return e;
 }
 
@@ -1066,7 +1068,7 @@ struct Maps {
 
 template <int kFmt, int kMode>
 static cudaError_t launch_many(const GemmArgs& g, const Maps& m, Device d, cudaStream_t s) {
-  static bool done[64] = {};
+  static std::atomic<bool> done[64] = {};
   auto kernel = gemm_pair_kernel<kFmt, kMode>;
   using S = Smem<kFmt, kMode>;
   static_assert(sizeof(S) + 1024 <= 232448, "shared memory of the stages");
@@ -1082,7 +1084,7 @@ static cudaError_t launch_many(const GemmArgs& g, const Maps& m, Device d, cudaS
 
 template <int kFmt, int kMode, int NT, int kRows, bool kRaw>
 static cudaError_t launch_few(const GemmArgs& g, const Maps& m, Device d, cudaStream_t s) {
-  static bool done[64] = {};
+  static std::atomic<bool> done[64] = {};
   auto kernel = gemm_few_kernel<kFmt, kMode, NT, kRows, kRaw>;
   using S = FewSmem<kFmt, NT>;
   static_assert(2 * (sizeof(S) + 2048) <= 228 * 1024, "two CTAs an SM");
@@ -1095,11 +1097,12 @@ static cudaError_t launch_few(const GemmArgs& g, const Maps& m, Device d, cudaSt
   // K in as many parts as clusters of that many CTAs can all run at once, and in no more than make the longest part
   // shorter. Clusters that do not all fit cost a second wave: 72 tiles in 4 parts (70 clusters of 4 fit) took 7.4 us,
   // in 2 parts 5.0 (N 9216, K 3072, one row).
-  static int room[64][9] = {};
+  static std::atomic<int> room[64][9] = {};
   const int dev = d.id >= 0 && d.id < 64 ? d.id : 0;
   int splits = 1;
   for (int n = 2; n <= 8 && n <= stages; ++n) {
-    if (room[dev][n] == 0) {
+    int fit = room[dev][n].load(std::memory_order_relaxed);
+    if (fit == 0) {
       cudaLaunchConfig_t c = {};
       cudaLaunchAttribute at;
       at.id = cudaLaunchAttributeClusterDimension;
@@ -1113,9 +1116,10 @@ static cudaError_t launch_few(const GemmArgs& g, const Maps& m, Device d, cudaSt
       // the query counts one CTA an SM here where shared memory, registers and TMEM hold two
       int blocks = 1;
       if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, kFewThreads, bytes) != cudaSuccess) cudaGetLastError();
-      room[dev][n] = blocks >= 2 ? clusters : 2 * clusters;
+      fit = blocks >= 2 ? clusters : 2 * clusters;
+      room[dev][n].store(fit, std::memory_order_relaxed);
     }
-    if (static_cast<int64_t>(n_tiles) * m_tiles <= room[dev][n]) splits = n;
+    if (static_cast<int64_t>(n_tiles) * m_tiles <= fit) splits = n;
   }
   const int share = (stages + splits - 1) / splits;
   splits = (stages + share - 1) / share;

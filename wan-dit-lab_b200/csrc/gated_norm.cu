@@ -21,6 +21,8 @@
 // store the first is 12.0. Slower: sums in float64 from the threads on (14.7 us for the first), three or four CTAs an SM
 // with fewer registers (19.8, 24), 192 or 128 threads a row with two or three chunks each (16.4, 18.4; the second 45.7 at
 // best), the modulation in shared memory (15.0), rows through a ring of bulk copies in shared memory (15.0 and 46.8).
+#include <atomic>
+
 #include "fp4.cuh"
 #include "fp4.h"
 
@@ -290,17 +292,19 @@ __global__ void __launch_bounds__(kThreads) gated_norm_kernel(const GatedNormArg
 // As many CTAs as fit the device (asked once per device), each with an equal share of neighbouring rows.
 template <typename TX, typename TY, int kThreads, int kChunks>
 static cudaError_t launch_rows(const GatedNormArgs& a, cudaStream_t s) {
-  static int room[64] = {};
+  static std::atomic<int> room[64] = {};
   auto kernel = gated_norm_kernel<TX, TY, kThreads, kChunks>;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-  if (room[dev] == 0) {
+  int fit = room[dev].load(std::memory_order_relaxed);
+  if (fit == 0) {
     int blocks = 1, sms = 148;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, kThreads, 0) != cudaSuccess) cudaGetLastError();
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    room[dev] = (blocks < 1 ? 1 : blocks) * sms;
+    fit = (blocks < 1 ? 1 : blocks) * sms;
+    room[dev].store(fit, std::memory_order_relaxed);
   }
-  return launch_dependent(kernel, dim3(a.M < room[dev] ? a.M : room[dev]), kThreads, s, a);
+  return launch_dependent(kernel, dim3(a.M < fit ? a.M : fit), kThreads, s, a);
 }
 
 cudaError_t gated_norm_launch(const GatedNormArgs& a, cudaStream_t s) {
