@@ -361,3 +361,25 @@ def test_tiles_of_the_many_row_product(tmp_path):
                     str(source), "-o", str(exe)], check=True)
     run = subprocess.run([str(exe)], capture_output=True, text=True)
     assert run.returncode == 0 and run.stdout == "ok\n", run.stderr
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+def test_a_cast_leaves_the_scales_and_the_bias(fmt):
+    from wan_dit_lab_b200.quantization import fp4
+    g = torch.Generator().manual_seed(0)
+    layer = lambda N, K: fp4.PackedFp4Linear(  # noqa: E731
+        torch.randint(0, 256, (N, K // 2), dtype=torch.uint8, generator=g),
+        torch.randint(0, 127, (N, K // fp4.BLOCK[fmt]), dtype=torch.uint8, generator=g),
+        torch.rand(1, generator=g) if fmt == "nvfp4" else None, torch.randn(N, generator=g), 0.1 if fmt == "nvfp4" else None)
+    mlp = fp4.PackedFp4GeluMLP(layer(96, 64), layer(32, 96))
+    model = torch.nn.Sequential(torch.nn.Linear(4, 4), mlp)
+    want = {name: t.clone() for name, t in mlp.state_dict().items()}
+    for cast in (lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(), lambda m: m.to("cpu", torch.bfloat16)):
+        assert cast(model) is model
+        now = mlp.state_dict()
+        assert set(now) == set(want)
+        for name, t in want.items():
+            assert now[name].dtype == t.dtype and torch.equal(now[name], t), name
+    assert model[0].weight.dtype == torch.bfloat16  # what is not FP4 was cast
+    for t in model.to("meta")[1].state_dict().values():
+        assert t.is_meta and t.dtype in (torch.uint8, torch.float32)

@@ -402,6 +402,17 @@ class PackedFp4Linear(torch.nn.Module):
         self.register_buffer("bias", bias)
         self.register_buffer("input_scale", one(input_scale))
 
+    def _apply(self, fn, recurse=True):
+        """Moves as any module's; a cast of a model to another dtype leaves the scales and the bias as they are (they are
+        numbers of the format and the epilogue's float32, not activations)."""
+        kept = {name: getattr(self, name) for name in ("tensor_scale", "input_scale", "bias")}
+        super()._apply(fn, recurse)
+        for name, old in kept.items():
+            new = getattr(self, name)
+            if old is not None and new.dtype is not old.dtype:
+                setattr(self, name, old.to(new.device))
+        return self
+
     def rows(self):
         return Rows(self.codes, self.tiles, self.fmt, self.tensor_scale)
 
