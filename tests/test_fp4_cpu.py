@@ -383,3 +383,33 @@ def test_a_cast_leaves_the_scales_and_the_bias(fmt):
     assert model[0].weight.dtype == torch.bfloat16  # what is not FP4 was cast
     for t in model.to("meta")[1].state_dict().values():
         assert t.is_meta and t.dtype in (torch.uint8, torch.float32)
+
+
+def test_forward_mode_tangents_are_refused(fake):
+    """Dual tensors do not require a gradient; a kernel would drop their tangents. Under no_grad too, as torch has it."""
+    from torch.autograd import forward_ad
+
+    from wan_dit_lab_b200 import _native
+    from wan_dit_lab_b200.kernels.gated_norm import gated_norm
+    from wan_dit_lab_b200.quantization import fp4
+    w, rows, w2 = fake_rows(96, 64), fake_rows(6, 64), fake_rows(32, 96)
+    x, y, v = cuda(6, 64), cuda(6, 96), cuda(96)
+    with forward_ad.dual_level():
+        d = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        calls = [
+            lambda: fp4.quantize_rows(d(x)), lambda: fp4.quantize_rows(x, "nvfp4", d(cuda(1))), lambda: fp4.fp4_linear(d(x), w),
+            lambda: fp4.fp4_linear(d(cuda(6, 66))[:, 1:65], w),  # (a copy is read)
+            lambda: fp4.fp4_linear(rows, w, d(v)), lambda: fp4.fp4_linear(rows, w, residual=d(y)),
+            lambda: fp4.fp4_linear(rows, w, residual=y, gate=d(v)), lambda: fp4.fp4_linear(rows, w, residual=y, out=d(y)),
+            lambda: fp4.fp4_linear(x, w, input_scale=d(cuda(1))), lambda: fp4.fp4_gelu_mlp(d(x), w, None, w2, None),
+            lambda: fp4.fp4_gelu_mlp(rows, w, d(v), w2, None), lambda: fp4.fp4_gelu_mlp(rows, w, None, w2, d(cuda(32))),
+            lambda: fp4.fp4_gelu_mlp(rows, w, None, w2, None, hidden_scale=d(cuda(1))), lambda: gated_norm(d(x)),
+            lambda: gated_norm(x, d(x)), lambda: gated_norm(x, x, d(cuda(64))), lambda: gated_norm(x, shift=d(cuda(64))),
+            lambda: gated_norm(x, scale=d(cuda(64))), lambda: gated_norm(x, weight=d(cuda(64))),
+            lambda: gated_norm(x, bias=d(cuda(64))), lambda: gated_norm(x, out="nvfp4", tensor_scale=d(cuda(1)))]
+        for call in calls:
+            with pytest.raises(ValueError, match="inference-only"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="inference-only"):
+                call()
+        _native.refuse_gradients("an ordinary tensor inside the level is not", x, None)

@@ -10,6 +10,7 @@ import struct
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIBRARY = Path(__file__).resolve().parent / "libwdl_b200.so"
 
@@ -149,6 +150,16 @@ def elsewhere(device):
 def raw_stream(device):
     """The current stream of a tensor's device as the library takes it, without the Stream object that stream() makes."""
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def refuse_gradients(what, *tensors):
+    """Refuses tensors (None among them) that autograd would follow: what requires a gradient where gradients are recorded,
+    and dual tensors of forward mode, whose tangents a kernel would drop (torch.no_grad does not turn these off)."""
+    grad, dual = torch.is_grad_enabled(), forward_ad._current_level >= 0
+    if grad or dual:
+        for t in tensors:
+            if t is not None and (grad and t.requires_grad or dual and forward_ad.unpack_dual(t).tangent is not None):
+                raise ValueError(f"{what} inference-only")
 
 
 def rows16(x):

@@ -63,10 +63,7 @@ def gated_norm(x, y=None, gate=None, *, weight=None, bias=None, shift=None, scal
         with torch.cuda.device(dev):
             return gated_norm(x, y, gate, weight=weight, bias=bias, shift=shift, scale=scale, eps=eps, kind=kind, out=out,
                               tensor_scale=tensor_scale, inplace=inplace)
-    if torch.is_grad_enabled():
-        for t in (x, y, gate, weight, bias, shift, scale):
-            if t is not None and t.requires_grad:
-                raise ValueError("gated_norm is inference-only")
+    _native.refuse_gradients("gated_norm is", x, y, gate, weight, bias, shift, scale)
     if y is None:
         if gate is not None or inplace:
             raise ValueError("gate and inplace belong to a branch y")

@@ -14,6 +14,7 @@ Inference only, like the rest of the package. No counterpart in the reference, w
 """
 
 import torch
+from torch.autograd import forward_ad
 
 from wan_dit_lab_b200 import _native
 
@@ -106,10 +107,7 @@ def _format(fmt):
 
 
 def _inference_only(*tensors):
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise ValueError("the FP4 operators are inference-only")
+    _native.refuse_gradients("the FP4 operators are", *tensors)
 
 
 def _tensor_scale(t, fmt, device, name="tensor scale"):
@@ -121,7 +119,7 @@ def _tensor_scale(t, fmt, device, name="tensor scale"):
         raise TypeError(f"the {name} must be one float32 number")
     if t.device != device:
         raise ValueError(f"the {name} must be on the operands' device")
-    if t.requires_grad:
+    if t.requires_grad or forward_ad._current_level >= 0:
         _inference_only(t)
     return t
 
@@ -168,7 +166,7 @@ def quantize_rows(x, fmt="nvfp4", tensor_scale=None):
     """Rows of x [M, K] (bfloat16, float16 or float32, CUDA, K a multiple of 32) in FP4: a Rows. tensor_scale (nvfp4):
     a float32 tensor of one element, read on the device."""
     code = _format(fmt)
-    if x.requires_grad:
+    if x.requires_grad or forward_ad._current_level >= 0:
         _inference_only(x)
     shape = x.shape
     if len(shape) != 2:
@@ -299,8 +297,7 @@ def fp4_linear(x, weight, bias=None, *, input_scale=None, dtype=torch.bfloat16, 
         with torch.cuda.device(device):
             return fp4_linear(x, weight, bias, input_scale=input_scale, dtype=dtype, residual=residual, gate=gate, out=out)
     rows, x2, lead, t = _input(x, w, input_scale)
-    if torch.is_grad_enabled():
-        _inference_only(x2, bias, residual, gate, out)
+    _inference_only(x2, bias, residual, gate, out)
     N, K = w.shape
     M = (rows or x2).shape[0]
     bias = _bias(bias, N, device)
@@ -340,8 +337,7 @@ def fp4_gelu_mlp(x, weight1, bias1, weight2, bias2, *, input_scale=None, hidden_
             return fp4_gelu_mlp(x, weight1, bias1, weight2, bias2, input_scale=input_scale, hidden_scale=hidden_scale,
                                 dtype=dtype, residual=residual, gate=gate, out=out)
     rows, x2, lead, t = _input(x, w1, input_scale)
-    if torch.is_grad_enabled():
-        _inference_only(x2, bias1, bias2, residual, gate, out)
+    _inference_only(x2, bias1, bias2, residual, gate, out)
     (H, K), N, fmt = w1.shape, w2.shape[0], w1.fmt
     if w2.fmt != fmt or w2.device != device or w2.shape[1] != H:
         raise ValueError(f"weight2 must have {H} columns, in weight1's format and on its device")
