@@ -198,3 +198,52 @@ def test_bad_and_extreme_rows_stay_their_own(kind, out):
     for row in (340, 341):
         assert torch.equal(got[row], only_shift)
     assert torch.allclose(got[699], only_shift, rtol=0, atol=0 if isinstance(out, str) else 1e-30)
+
+
+@pytest.mark.parametrize("K", [12288, 16384])
+def test_sums_over_long_rows_are_not_rounded_on_the_way(K):
+    """Four values, each over a quarter of the row, whose float32 sums from left to right would round down three times,
+    while the row's mean 1 + 2^-23 is a float32 number: the values' distances from it come out exactly, whichever columns
+    they lie in."""
+    from wan_dit_lab_b200.kernels.gated_norm import gated_norm
+    step = 2.0 ** -23
+    quarter = torch.tensor([1 + step, 1.0, 1 + step, 1 + 2 * step], dtype=torch.float64)
+    for x in (quarter.repeat_interleave(K // 4), quarter.repeat_interleave(8).repeat(K // 32), quarter.repeat(K // 4)):
+        h = gated_norm(x.float().to(DEV)[None], eps=0.0, out=torch.float32)[1][0].double().cpu()
+        want = (x - (1 + step)) / (step / 2 ** 0.5)  # the root of the mean square, (0 + 1 + 0 + 1) / 4 steps
+        # the squares and their sums are exact; the root and the quotient round once each
+        assert ((h - want).abs() <= 2.0 ** -24 * 2.02 * want.abs()).all()
+
+
+def statistics_case(data, K, g):
+    x = torch.randn(3, K, generator=g)
+    if data == "offset":
+        return x + 1000.0
+    if data == "outliers":  # far larger values that cancel, an ordinary mean
+        x[:, ::8] = 30000.0 * torch.sign(torch.randn(3, -(-K // 8), generator=g))
+        return x
+    return 1000.0 * x - (1000.0 * x).double().mean(-1, keepdim=True).float()  # the mean cancels to nearly nothing
+
+
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("data", ["offset", "outliers", "centred"])
+@pytest.mark.parametrize("K", [1024, 3072, 4096, 5120, 8192, 16384])
+def test_statistics_of_rows_far_from_standard(kind, data, K):
+    """Bound, in halves of a float32 step s = 2^-24. The float32 sums of 64 columns (8 from 4097 columns on) round 6 (3)
+    times, relative to the magnitudes of what they add, the sum and its division once each: the mean's error is e <= (6
+    mean|x| + 2 |mean|) s. It shifts every value; of the mean square it changes e^2 alone, the values' sum being zero. The
+    subtraction rounds once; the mean square takes that twice, its squares' and sums' roundings (7, or 4) and its own
+    (2), eps's sum one more, half of which reach the root; the root and the quotient round once each."""
+    from wan_dit_lab_b200.kernels.gated_norm import gated_norm
+    s, sums = 2.0 ** -24, 6 if K <= 4096 else 3
+    x = statistics_case(data, K, generator(K))
+    h = f64(gated_norm(x.to(DEV), kind=kind, out=torch.float32)[1])
+    v = f64(x)
+    _, u = oracle.norm(v, kind=kind)
+    e = sub = np.zeros((3, 1))
+    if kind == "layer":
+        mean = v.mean(-1, keepdims=True)
+        root = np.sqrt(((v - mean) ** 2).mean(-1, keepdims=True) + 1e-6)
+        e, sub = (sums * np.abs(v).mean(-1, keepdims=True) + 2 * np.abs(mean)) * s / root, 1
+    relative = (sub + (2 * sub + sums + 1 + 2 + 1) / 2 + 2) * s + e ** 2 / 2
+    assert (np.abs(h - u) <= 1.01 * (e + relative * np.abs(u))).all(), float((np.abs(h - u) / (e + relative * np.abs(u))).max())

@@ -11,9 +11,11 @@
 // bound the kernel. Bytes: x and y read once, x' and h written once.
 //
 // Every step is one float32 operation, rounded to nearest (gate y, then the sum; the division by the root, not a product
-// with its inverse), and the two statistics are exact to a fraction of float32's last bit (sums of 64 columns in float32,
-// of these in float64) before they are rounded: a value of h next to a border of the FP4 codes falls to one side or the
-// other by its last bit, and an error of the row's statistics moves all of the row's values.
+// with its inverse). Of the two statistics only the sums of 64 columns are float32 (of 8 in rows of several chunks), the sums
+// of these are float64: a statistic's error before its own rounding is at most 6 (3) half steps of float32 relative to the
+// mean magnitude of what it adds, and mostly a fraction of one, since the parts' errors differ. A value of h next to a border
+// of the FP4 codes falls to one side or the other by its last bit, and an error of the row's statistics moves all of the
+// row's values.
 //
 // What bounds it: instructions and the chain of two reductions a row, not HBM, at the block widths. Measured on a B200 with
 // gate, LayerNorm and modulation, rows of 3072: 1392 rows (x float32, y bf16) into NVFP4 14.3 us; 7040 rows (bf16, 8 groups)
@@ -22,6 +24,7 @@
 // with fewer registers (19.8, 24), 192 or 128 threads a row with two or three chunks each (16.4, 18.4; the second 45.7 at
 // best), the modulation in shared memory (15.0), rows through a ring of bulk copies in shared memory (15.0 and 46.8).
 #include <atomic>
+#include <type_traits>
 
 #include "fp4.cuh"
 #include "fp4.h"
@@ -79,15 +82,17 @@ __device__ __forceinline__ void store8(float* p, const Eight& v) {
   reinterpret_cast<ulonglong2*>(p)[1] = make_ulonglong2(v.p[2], v.p[3]);
 }
 
-// The CTA's sum over the row, in a fixed order, rounded to float32 and divided by K. red: one number a warp, not the array
-// of the call before.
-template <int kWarps>
-__device__ __forceinline__ float block_mean(float part, double* red, float K, float inverse_k) {
+// The CTA's sum over the row, in a fixed order, rounded to float32 and divided by K. part: a thread's 8 columns in float32,
+// which 8 threads add up to 64 of them, or the float64 sum of its chunks. red: one number a warp, not the array of the call
+// before.
+template <int kWarps, typename Sum>
+__device__ __forceinline__ float block_mean(Sum part, double* red, float K, float inverse_k) {
+  constexpr int kFirst = sizeof(Sum) == 4 ? 8 : 1;
 #pragma unroll
-  for (int o = 1; o < 8; o *= 2) part += __shfl_xor_sync(0xFFFFFFFFu, part, o);
+  for (int o = 1; o < kFirst; o *= 2) part += __shfl_xor_sync(0xFFFFFFFFu, part, o);
   double v = part;
 #pragma unroll
-  for (int o = 8; o < 32; o *= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  for (int o = kFirst; o < 32; o *= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   double s[kWarps];
@@ -139,6 +144,7 @@ __device__ __forceinline__ void store_fp4(const GatedNormArgs& a, int m, int k, 
 template <typename TX, typename TY, int kThreads, int kChunks>
 __global__ void __launch_bounds__(kThreads) gated_norm_kernel(const GatedNormArgs a) {
   constexpr int kWarps = kThreads / 32;
+  using Sum = std::conditional_t<kChunks == 1, float, double>;
   __shared__ double red[3][kWarps];  // in turn: two sums a row, so that none is written again before all have read it
   grid_dependency_wait();
   grid_dependents_launch();
@@ -185,7 +191,7 @@ __global__ void __launch_bounds__(kThreads) gated_norm_kernel(const GatedNormArg
       if (kChunks == 1) kept = modulation(group, t * 8);
     }
     Eight v[kChunks];
-    float s = 0.f;
+    Sum s = 0;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       const int k = (c * kThreads + t) * 8;
@@ -217,7 +223,7 @@ __global__ void __launch_bounds__(kThreads) gated_norm_kernel(const GatedNormArg
     turn = turn == 2 ? 0 : turn + 1;
     if (!a.rms) {
       const uint64_t minus = pack2(-var, -var);
-      s = 0.f;
+      s = 0;
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
         if ((c * kThreads + t) * 8 >= K) continue;
