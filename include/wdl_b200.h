@@ -417,7 +417,9 @@ int wdl_fp4_dequantize_rows(const uint8_t* codes, const uint8_t* scales, int M, 
                             const float* tensor_scale, void* out, int out_dtype, int64_t ldo, void* stream);
 
 /* out [M, N] (out_dtype, row stride ldo) = a [M, K] w [N, K]^T + bias[n] from FP4 operands of one format (the tensor
- * cores' block-scaled MMA, float32 accumulation, one rounding at the end). bias f32 [N] nullable; any M >= 0, N >= 1. */
+ * cores' block-scaled MMA, float32 accumulation, one rounding at the end). bias f32 [N] nullable; any M >= 0, N >= 1.
+ * The operands' tensor scales are multiplied first, in float32: their product has to be a normal number (outside of about
+ * 1e-38 to 3e38 in magnitude results lose their bits, or become 0, infinite or NaN). */
 int wdl_fp4_gemm(const wdl_fp4_rows* a, const wdl_fp4_rows* w, const float* bias, int M, int N, int K, void* out,
                  int out_dtype, int64_t ldo, void* stream);
 
@@ -427,8 +429,8 @@ int wdl_fp4_gemm(const wdl_fp4_rows* a, const wdl_fp4_rows* w, const float* bias
 int wdl_fp4_gemm_rows_per_cta(int M, int N, int K, int sms);
 
 /* out [M, N] f32 = residual + gate * (a w^T + bias): the gated residual update of a block. gate [groups, ld_gate] f32
- * (nullable: 1): row m takes group m / (M / groups), M a multiple of groups. out may be residual itself (the same
- * rows), and otherwise overlaps nothing that is read. */
+ * (nullable: 1): row m takes group m / (M / groups), M a multiple of groups. out may be residual itself (all of the same
+ * rows), and otherwise overlaps nothing that is read (no gate or bias out of its rows). */
 int wdl_fp4_gemm_residual(const wdl_fp4_rows* a, const wdl_fp4_rows* w, const float* bias, const float* gate, int groups,
                           int64_t ld_gate, const float* residual, int64_t ldr, int M, int N, int K, float* out,
                           int64_t ldo, void* stream);
@@ -465,8 +467,8 @@ int wdl_fp4_gelu_mlp(const void* x, int x_dtype, int64_t ldx, const float* x_sca
  * in float32. x, x_out bf16 or f32 (x_dtype); y bf16 or f32; h in `out`: WDL_BF16, WDL_F16, WDL_F32 (row stride ldh), or
  * WDL_OUT_NVFP4 / WDL_OUT_MXFP4: h codes, h_scales their tiles. gate, shift, scale f32 rows [groups, ld_*]: row m takes
  * group m / (M / groups). K a multiple of 8 (FP4: 32), at most 16384; rows and vectors 16-byte aligned. x_out may be x,
- * and h may be y where row strides and types agree; otherwise they overlap nothing that is read. models/block.py:75-79 (residual update, norm1 / norm2 / norm3 and
- * their modulation). */
+ * and h may be y where row strides and types agree; otherwise they overlap nothing that is read (no modulation row, weight
+ * or bias out of their rows). models/block.py:75-79 (residual update, norm1 / norm2 / norm3 and their modulation). */
 #define WDL_OUT_NVFP4 3
 #define WDL_OUT_MXFP4 4
 typedef struct wdl_gated_norm_args {

@@ -340,8 +340,9 @@ __device__ __forceinline__ uint32_t elect_one() {
 
 // ---------------------------------------------------------------------------------------------------------------
 // CTA pairs (a cluster of two CTAs on the two SMs of a TPC): 2-SM MMAs, whose operands and accumulator are split
-// between the pair. Every tcgen05 instruction of a kernel that uses them takes .cta_group::2. No multicast form is
-// used: a signal the peer needs is relayed by a remote mbarrier arrive.
+// between the pair. Every tcgen05 instruction of a kernel that uses them takes .cta_group::2. No load is multicast: each
+// CTA brings its own share. A signal the peer needs is a remote mbarrier arrive, or (fp4_gemm.cu) a commit that arrives in
+// both CTAs.
 
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;

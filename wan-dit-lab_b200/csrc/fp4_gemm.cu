@@ -1167,7 +1167,7 @@ static bool make_maps(Maps& m, const GemmArgs& g, int few) {
 // Up to 64 rows the few-row kernel is the faster one (N 14336, K 3072: 8.2 against 8.9 us at 64 rows, 9.5 against 8.5 at
 // 96). Beyond, 64 rows a CTA where these are few enough for K to be split, two thirds of the SMs (128 rows: 4.4 against 5.5
 // us for N 512, K 1024, 7.2 against 7.9 for N 3072, K 3072, 5.7 against 13.2 for N 512, K 8192; 256 rows, 96 CTAs: 7.7
-// against 7.9 for N 3072, K 3072). Where K is long, at most half as many: CTAs of 128 rows read w less often (K 14336, N
+// against 7.9 for N 3072, K 3072). Where K is long, two thirds as many: CTAs of 128 rows read w less often (K 14336, N
 // 3072: 10.9 against 12.0 us at 128 rows, 13.7 against 13.0 at 160), and are taken as long as their parts find room beside
 // each other (18.1 against the many-row kernel's 21.5 us at 384 rows, 22.2 against 21.5 at 512).
 int gemm_rows_per_cta(int M, int N, int K, int sms) {

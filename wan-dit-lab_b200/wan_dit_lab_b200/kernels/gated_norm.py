@@ -41,8 +41,7 @@ def gated_norm(x, y=None, gate=None, *, weight=None, bias=None, shift=None, scal
     x). kind "layer" (LayerNorm) or "rms" (x / sqrt(mean x^2 + eps)); weight and bias [K]; gate, shift and scale [K],
     or [G, K] for G groups of consecutive rows (a modulation per frame). out: h's dtype (bfloat16, float16, float32), or
     "nvfp4" (with tensor_scale) or "mxfp4" for a fp4.Rows. inplace: x' is written over x (y may be x, but nothing else may
-    overlap it). K a multiple of 8 (FP4: 32),
-    at most 16384."""
+    overlap it). K a multiple of 8 (FP4: 32), at most 16384."""
     if kind not in ("layer", "rms"):
         raise ValueError("kind must be 'layer' or 'rms'")
     if out not in _OUT:

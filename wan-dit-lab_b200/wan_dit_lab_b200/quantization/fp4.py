@@ -10,7 +10,8 @@ format does not give the other's results.
 
 in float32, rounded to nearest even, magnitudes above 6 become 6. A block with an infinity or a NaN becomes NaN as a
 whole. Codes are two a byte (low nibble: the even channel); scales lie in the tensor cores' tiles (tile_scales).
-Inference only, like the rest of the package. No counterpart in the reference, whose 4-bit layers are INT4.
+Inference only, like the rest of the package: inputs that require a gradient or carry a forward-mode tangent are refused.
+No counterpart in the reference, whose 4-bit layers are INT4.
 """
 
 import torch
@@ -290,7 +291,8 @@ def fp4_linear(x, weight, bias=None, *, input_scale=None, dtype=torch.bfloat16, 
     input_scale, nvfp4's tensor scale) or a Rows already; weight a Rows [N, K]; bias [N]. y [..., N] in dtype.
     With residual [..., N] float32 the gated residual update residual + gate * y instead, float32: gate [N], or [G, N]
     for G groups of consecutive rows (a modulation per frame), None for 1; out: where to write it (the residual itself
-    to update it in place)."""
+    to update it in place; nothing else that is read may overlap it). nvfp4: the two tensor scales are multiplied first, in
+    float32, and their product has to be a normal number there."""
     w = _weight(weight, "weight")
     device = w.device
     if _native.elsewhere(device):
