@@ -99,6 +99,28 @@ def test_gelu_mlp_of_many_rows(fmt, first, second, M, K, H, N):
     small.test_gelu_mlp(fmt, M, K, H, N)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("H", range(256 + 32, 512 + 32, 32))
+def test_hidden_layers_of_many_rows_that_end_anywhere_in_a_tile(fmt, H):
+    """Every width of the last tile: codes, scales, zeros in the padding of the last tile of scales, and the scales of rows
+    behind the last left as they were."""
+    from wan_dit_lab_b200 import _native
+    from wan_dit_lab_b200.quantization import fp4
+    takes(0, 3300, H, 96)
+    small.test_gelu_mlp(fmt, 3300, 96, H, 24)
+    x = fp4.quantize_rows(activations(3300, 96, 170), fmt)
+    w, _ = weight_rows(H, 96, fmt, 171)
+    tiles = torch.full(fp4.scale_tiles(3300, H, fmt), 0xAB, dtype=torch.uint8, device=DEV)
+    codes = torch.empty(3300, H // 2, dtype=torch.uint8, device=DEV)
+    _native.check(_native.lib().wdl_fp4_gemm_gelu(x._operand, w._operand, None, 3300, H, 96, None, codes.data_ptr(),
+                                                  tiles.data_ptr(), _native.stream()))
+    blocks = H // fp4.BLOCK[fmt]
+    by_row = fp4.untile_scales(tiles, 3328, -(-blocks // 4) * 4)
+    want = small.hidden_of(x, w, None, fmt, None)
+    assert torch.equal(by_row[:3300, :blocks], fp4.untile_scales(want.scales, 3300, blocks)) and torch.equal(codes, want.codes)
+    assert not by_row[:3300, blocks:].any() and (by_row[3300:] == 0xAB).all()
+
+
 @pytest.mark.parametrize("M", [1700, 1665])
 def test_a_square_layer_of_many_rows_onto_its_own_input(M):
     takes(0, M, 512, 512)
